@@ -124,8 +124,6 @@ def prepare(case, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     c, op = case, case["op"]
     s = {"case": c}
-    if own:
-        _package()
     if op == "quantize":
         w = torch.randn(c["N"], c["K"], generator=g, device="cuda") / math.sqrt(c["K"])
         s["w"] = w.to(DTYPES[c["dtype"]])
@@ -150,6 +148,7 @@ def prepare(case, seed):
             top = p.topk(c["k"], dim=-1)
             s["ids"], s["weights"] = top.indices.int(), top.values
     if own:  # the weights in the framework's layout, as a program lays them out once when it loads them
+        _package()
         from sb200 import group4, moe, ternary
 
         def packed(m):
@@ -175,7 +174,8 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------
 
 def _run_own(s):
-    from sb200 import group4  # on the import path since prepare()
+    _package()
+    from sb200 import group4
     c, op = s["case"], s["case"]["op"]
     if op == "quantize":
         m, values = group4.quantize(s["w"], group=c["group"], symmetric=not c["zeros"], values=True)

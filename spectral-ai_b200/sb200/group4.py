@@ -112,6 +112,8 @@ class Group4Matrix:
                 or data.numel() != need:
             raise RuntimeError(f"{self.count} matrices [{N}, {K}] in groups of {group} are {need} contiguous bytes, got "
                                f"{data.dtype} {tuple(data.shape)}")
+        if data.data_ptr() % 16:
+            raise RuntimeError("data must start on a 16-byte boundary")
         self.data, self.device = data, data.device
         self.desc = _lib.Group4(data.data_ptr(), self.K, self.N, self.count, self.group, int(self.has_zeros))
         self.ref = C.byref(self.desc)
@@ -155,11 +157,12 @@ class Group4Matrix:
         return m
 
     def _rows(self, flat: torch.Tensor, block: int, offset: int) -> torch.Tensor:
-        """Scales or zero points (``flat``: the data as their type, ``block`` of it to a
-        block, theirs from ``offset``) row-major: [count * N, groups], one copy."""
+        """Scales or zero points (``flat``: the data as their type, which may begin anywhere
+        in its storage, ``block`` of it to a block, theirs from ``offset``) row-major:
+        [count * N, groups], one copy."""
         tiles, chunks, per = (self.N + 15) // 16, (self.K + 127) // 128, 128 // self.group
         t = flat.as_strided((self.count, tiles, 2, 8, chunks, per), (tiles * chunks * block, chunks * block, 1, 2, block, 16),
-                            offset)
+                            flat.storage_offset() + offset)
         t = t.reshape(self.count, tiles * 16, chunks * per)[:, :self.N, :-(-self.K // self.group)]
         return t[0] if self.count == 1 else t.reshape(self.count * self.N, -1)
 

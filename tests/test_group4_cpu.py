@@ -167,3 +167,30 @@ def test_restated_quantiser():
     assert (scales, zeros) == ([[1.0]], [[1]]) and codes.tolist() == [[0, 15, 1, 1]]
     v = og.values(codes, scales, zeros, 32)
     assert v.tolist() == [[-1.0, 14.0, 0.0, 0.0]]
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_scales_of_data_inside_a_larger_buffer(group, zeros):
+    """Scales and zero points are read from the matrix's own bytes, wherever they begin."""
+    N, K, count = 33, 300, 2
+    nbytes = count * _lib.load().sb_group4_matrix_bytes(K, N, group, int(zeros))
+    data = torch.from_numpy(np.random.default_rng(group).integers(0, 256, nbytes).astype(np.uint8))
+
+    def matrix_on(d):
+        m = group4.Group4Matrix.__new__(group4.Group4Matrix)
+        m.N, m.K, m.group, m.count, m.has_zeros, m.data = N, K, group, count, zeros, d
+        return m
+
+    buffer = torch.zeros(nbytes + 4096, dtype=torch.uint8)
+    buffer[1040:1040 + nbytes] = data
+    whole, part = matrix_on(data), matrix_on(buffer[1040:1040 + nbytes])
+    assert torch.equal(part.scales.view(torch.int16), whole.scales.view(torch.int16))
+    # row 17 = 16 + 1 of the second matrix: tile 1, place 2 of each group's scales (after 1024 bytes of words)
+    block, per = 1024 + (48 if zeros else 32) * (128 // group), 128 // group
+    at = ((1 * 3 + 1) * 3 + 0) * block + 1024 + 2 * 2
+    assert part.scales[N + 17, 0].view(torch.int16) == data[at:at + 2].view(torch.int16)[0]
+    if zeros:
+        assert torch.equal(part.zeros, whole.zeros)
+        assert part.zeros[N + 17, 0] == data[((1 * 3 + 1) * 3) * block + 1024 + 32 * per + 2]
+    else:
+        assert part.zeros is None

@@ -358,3 +358,20 @@ def test_many_tokens_of_a_narrow_matrix(cuda_device, M, K, N, dtype):
     xd = x.double().cpu().numpy()
     ref, bound = og.product(xd, v, np.abs(xd) * (2.0 ** -24 if fp32 else 0), 3 if fp32 else 2)
     close(group4.linear(x, w), ref, bound, "linear")
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (128, False)])
+def test_data_inside_a_larger_buffer(cuda_device, group, zeros):
+    """A matrix whose bytes are a slice of a checkpoint's: products, values, scales and zero points."""
+    from sb200 import group4
+    m, _ = make(50, 300, group, zeros, cuda_device)
+    n = m.data.numel()
+    buffer = torch.full((n + 4096,), 255, dtype=torch.uint8, device=cuda_device)
+    buffer[1040:1040 + n] = m.data
+    part = group4.Group4Matrix(buffer[1040:1040 + n], 50, 300, group, zeros)
+    x = acts(5, 300, torch.bfloat16, cuda_device)
+    assert torch.equal(group4.linear(x, part), group4.linear(x, m))
+    assert torch.equal(part.dequantize(), m.dequantize()) and torch.equal(part.scales, m.scales)
+    assert (part.zeros is None) if not zeros else torch.equal(part.zeros, m.zeros)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        group4.Group4Matrix(buffer[1032:1032 + n], 50, 300, group, zeros)

@@ -198,6 +198,8 @@ class TernaryExperts:
         for t in (gate, up, down):
             if not t.is_cuda or t.dtype != torch.int8 or t.dim() != 3:
                 raise RuntimeError(f"ternary weights must be CUDA int8 [E,N,K], got {t.device} {t.dtype} {tuple(t.shape)}")
+        if len({t.device for t in (gate, up, down)}) > 1:
+            raise RuntimeError("gate, up and down must be on one device")
         E, I, H = gate.shape
         if tuple(up.shape) != (E, I, H) or tuple(down.shape) != (E, H, I):
             raise RuntimeError(f"gate {tuple(gate.shape)}, up {tuple(up.shape)} and down {tuple(down.shape)} are not "

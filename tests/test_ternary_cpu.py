@@ -104,3 +104,24 @@ def test_torch_packer_matches_host_packer():
         T = rng.integers(-1, 2, size=shape, dtype=np.int8)
         a = pack_device_torch(torch.from_numpy(T)).numpy().view(np.uint32)
         assert np.array_equal(a, pack_device(T))
+
+
+def test_from_tensors_refuses_weights_on_different_devices():
+    """Weights of two GPUs are refused before anything is packed: the kernels get raw pointers of one device."""
+    from sb200 import ternary
+
+    class OnGpu:
+        is_cuda, dtype = True, torch.int8
+
+        def __init__(self, shape, index):
+            self.shape, self.device = torch.Size(shape), torch.device("cuda", index)
+
+        def dim(self):
+            return len(self.shape)
+
+    E, I, H = 2, 3, 5
+    scales = torch.ones(E, I), torch.ones(E, I), torch.ones(E, H)
+    for devices in ((0, 1, 0), (0, 0, 1), (1, 0, 0)):
+        weights = [OnGpu(s, d) for s, d in zip(((E, I, H), (E, I, H), (E, H, I)), devices)]
+        with pytest.raises(RuntimeError, match="one device"):
+            ternary.TernaryExperts.from_tensors(*weights, *scales)

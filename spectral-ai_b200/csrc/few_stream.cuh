@@ -27,8 +27,8 @@
 //
 // Tokens are bf16 in T planes (x = sum of the planes): 1 for bf16 activations,
 // 3 for fp32 ones (8 bits each: 24 bits, fp32's mantissa), 2 or 3 for the hidden
-// state between two products.  Weights (code - zero, -15..15, or -1..1) and the
-// planes are exact in bf16, products exact, sums fp32.
+// state between two products.  Weights (2^-12 times code - zero, -15..15, or -1..1) and
+// the planes are exact in bf16, products exact, sums fp32.
 //
 // What shaped it (B200, warm, per kernel of a 1-token layer; the cycles are those of
 // the first version, before the change that the line names):
@@ -198,6 +198,9 @@ struct Group4W {
   static constexpr int PER = 128 / G;    // groups per chunk
   static constexpr int BLOCKS = G / 32;  // 32-K blocks per group
   static constexpr int SLOT = 1024 + 48 * PER;  // shared memory of a block
+  // Sums are in units of 2^12: weights enter as 2^-12 (code - zero), so that a group's sum
+  // before its scale, up to 15 x 128 tokens' values, overflows for no finite ones.
+  static constexpr float UNIT = 4096.f;
   const uint8_t* data;
   int chunks, tiles;  // per matrix: chunks of a row, row tiles
   int block;          // bytes of a block: 1024 + 32 PER, with zero points 1024 + 48 PER
@@ -221,11 +224,11 @@ struct Group4W {
     }
   }
 
-  // Pair j of a word (elements 2j, 2j + 1 in its halves) minus the zero point:
-  // OR-ing 2^7's exponent under the code gives 128 + code, exact in bf16, and
-  // `sub` holds 128 + zero twice.
+  // Pair j of a word (elements 2j, 2j + 1 in its halves) minus the zero point, over UNIT:
+  // OR-ing 2^-5's exponent over the code gives 2^-12 (128 + code), exact in bf16, and
+  // `sub` holds 2^-12 (128 + zero) twice.
   static __device__ __forceinline__ uint32_t pair(uint32_t w, int j, uint32_t sub) {
-    const uint32_t v = and_or(w >> (4 * j), 0x000F000Fu, 0x43004300u);
+    const uint32_t v = and_or(w >> (4 * j), 0x000F000Fu, 0x3D003D00u);
     const __nv_bfloat162 d =
         __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&sub));
     return *reinterpret_cast<const uint32_t*>(&d);
@@ -263,8 +266,8 @@ struct Group4W {
       uint32_t sub[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        sub[r][0] = __byte_perm(part.z[r][q], 0x43u, 0x4040u);  // bytes z, 0x43, z, 0x43
-        sub[r][1] = __byte_perm(part.z[r][q], 0x43u, 0x4141u);
+        sub[r][0] = __byte_perm(part.z[r][q], 0x3Du, 0x4040u);  // bytes z, 0x3D, z, 0x3D
+        sub[r][1] = __byte_perm(part.z[r][q], 0x3Du, 0x4141u);
       }
 #pragma unroll
       for (int i = 0; i < BLOCKS; ++i) {
@@ -310,7 +313,6 @@ struct Group4W {
       }
     }
   }
-  __device__ __forceinline__ float out_scale(int64_t) const { return 1.f; }
 };
 
 // ---------------------------------------------------------------------------
@@ -325,6 +327,7 @@ struct TernaryW {
   static constexpr bool BULK = false;
   static constexpr int ARRIVALS = 32;
   static constexpr int SLOT = 1024;
+  static constexpr float UNIT = 1.f;  // of the sums
   const uint32_t* words;
   const float* scales;
   int chunks, blocks;
@@ -701,10 +704,10 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS)
 #pragma unroll
           for (int r = 0; r < UT * 2; ++r) {  // the lane's rows c0 + g + 8 r
             const int ch = c0 + g + 8 * r, at = min(ch, N - 1);
-            float a = acc[GATEUP ? 0 : r / 2][i][q + (r & 1) * 2];
+            float a = acc[GATEUP ? 0 : r / 2][i][q + (r & 1) * 2] * W::UNIT;
             if constexpr (W::ROW_SCALES) a *= w0.out_scale(base + at);
             if constexpr (GATEUP) {
-              float b = acc[1][i][q + (r & 1) * 2];
+              float b = acc[1][i][q + (r & 1) * 2] * W::UNIT;
               if constexpr (W::ROW_SCALES) b *= w1.out_scale(base + at);
               if (ch < hidden.ld)  // columns N .. ld: zero
                 store_hidden<TH>(hidden.h + line + ch, hidden.plane, ch < N ? a : 0.f, ch < N ? b : 0.f);

@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 1) moe_few_sum_kernel(W wd, Fe
     wd.template chunk<1>(now, c, FewTokens<TH, 1>(sx + first * TH * row_bytes, n, row_bytes, g, t), acc);
     const bool last = c + 1 == chunks;
     if (last || item + 1 == end) {
-      float sa = 1.f, sb = 1.f;
+      float sa = W::UNIT, sb = W::UNIT;
       if constexpr (W::ROW_SCALES) {
         sa = wd.out_scale((int64_t)e * H + min(r0 + g, H - 1));
         sb = wd.out_scale((int64_t)e * H + min(r0 + 8 + g, H - 1));

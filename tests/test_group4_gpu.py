@@ -375,3 +375,25 @@ def test_data_inside_a_larger_buffer(cuda_device, group, zeros):
     assert (part.zeros is None) if not zeros else torch.equal(part.zeros, m.zeros)
     with pytest.raises(RuntimeError, match="16-byte"):
         group4.Group4Matrix(buffer[1032:1032 + n], 50, 300, group, zeros)
+
+
+@pytest.mark.parametrize("M", [1, 20, 700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_group_sums_of_large_activations(cuda_device, M, dtype):
+    """A group's sum before its scale may be past fp32's range where the product is not:
+    128 weights of 15 x 2^-20 on activations of 2^126."""
+    from sb200 import group4
+    K, N = 256, 1000
+    w = group4.Group4Matrix.pack(torch.full((N, K), 15, dtype=torch.uint8, device=cuda_device),
+                                 torch.full((N, 2), 2.0 ** -20, device=cuda_device),
+                                 torch.zeros(N, 2, dtype=torch.uint8, device=cuda_device))
+    x = torch.full((M, K), 2.0 ** 126, dtype=dtype, device=cuda_device)
+    y = group4.linear(x, w, out_dtype=torch.float32)
+    assert (y == 15 * 2.0 ** 114).all()                    # every partial sum is a whole multiple of 2^106 below 2^118: exact
+    experts = group4.Group4Experts.pack(*({"codes": torch.full((1, n, k), 9, dtype=torch.uint8, device=cuda_device),
+                                           "scales": torch.full((1, n, -(-k // 128)), s, device=cuda_device)}
+                                          for n, k, s in ((128, K, 2.0 ** -100), (128, K, 2.0 ** -30), (K, 128, 2.0 ** -20))))
+    ids = torch.zeros(M, 1, dtype=torch.int32, device=cuda_device)
+    y = experts.forward_few(x * 2.0 ** -6, ids, torch.ones(M, 1, device=cuda_device))
+    # gate 2^28, and silu of it the same; up 2^98; 128 hidden values of 2^126 at 2^-20
+    assert (y == 2.0 ** 113).all()

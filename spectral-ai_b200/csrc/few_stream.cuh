@@ -449,12 +449,22 @@ __device__ __forceinline__ void few_bars_init(uint64_t* bars, int n) {
   fence_barrier_init();
 }
 
-// v as planes: bf16(v), bf16 of what that leaves, and so on (a non-finite v
-// leaves NaN in the second plane, so the token's results are non-finite).
+// v as planes: bf16(v), bf16 of what that leaves, and so on.  A finite v that bf16 would
+// round to infinity (from 3.39e38 on) has its first plane rounded towards zero, which
+// leaves the others no more than they hold; an infinite v is its first plane alone.
 template <int T>
 __device__ __forceinline__ void split_planes(float v, __nv_bfloat16 (&p)[T]) {
+  p[0] = __float2bfloat16_rn(v);
+  if (T > 1 && isinf(__bfloat162float(p[0]))) {
+    if (isinf(v))
+      v = 0.f;
+    else
+      v -= __bfloat162float(p[0] = __float2bfloat16_rz(v));
+  } else {
+    v -= __bfloat162float(p[0]);
+  }
 #pragma unroll
-  for (int i = 0; i < T; ++i) {
+  for (int i = 1; i < T; ++i) {
     p[i] = __float2bfloat16_rn(v);
     v -= __bfloat162float(p[i]);
   }

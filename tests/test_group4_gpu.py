@@ -397,3 +397,36 @@ def test_group_sums_of_large_activations(cuda_device, M, dtype):
     y = experts.forward_few(x * 2.0 ** -6, ids, torch.ones(M, 1, device=cuda_device))
     # gate 2^28, and silu of it the same; up 2^98; 128 hidden values of 2^126 at 2^-20
     assert (y == 2.0 ** 113).all()
+
+
+@pytest.mark.parametrize("M", [2, 20])
+def test_largest_and_infinite_fp32_values(cuda_device, M):
+    """fp32 values that bf16 rounds to infinity stay what they are, and an infinity stays one:
+    activations, and the hidden state of the gated MLP."""
+    from sb200 import group4
+    K, big = 128, torch.finfo(torch.float32).max
+    codes = torch.full((3, K), 8, dtype=torch.uint8, device=cuda_device)
+    codes[0, :], codes[1, 5], codes[2, 5:7] = 9, 9, 7     # row 0 meets every value, rows 1 and 2 the fifth (and sixth)
+    w = group4.Group4Matrix.pack(codes, torch.full((3, 1), 2.0 ** -10, device=cuda_device))
+    x = torch.zeros(M, K, device=cuda_device)
+    for value in (big, -big, 3.3962e38, -3.4e38):
+        x[:, 5] = value
+        # one product, all planes of it: exact
+        want = torch.tensor([1.0, 1.0, -1.0], dtype=torch.float64) * x[0, 5].item() * 2.0 ** -10
+        assert torch.equal(group4.linear(x, w).double().cpu(), want.expand(M, 3))
+    x[:, 5] = -torch.inf
+    y = group4.linear(x, w)
+    assert (y[:, 1] == -torch.inf).all() and (y[:, 2] == torch.inf).all()
+    # silu(g) u = g u where exp(-g) is lost beside 1
+    scale = lambda s, n: torch.tensor([[s]], device=cuda_device).expand(n, 1)  # noqa: E731
+    gate, up = (group4.Group4Matrix.pack(codes[1:2].expand(8, K), scale(s, 8)) for s in (1.0, 2.0 ** -64))
+    down = group4.Group4Matrix.pack(torch.full((K, 8), 9, dtype=torch.uint8, device=cuda_device), scale(2.0 ** -10, K))
+    x.zero_()
+    x[:, 5] = 2.0 ** 96 * (2.0 - 2.0 ** -23)              # h = (2 - 2^-23)^2 2^128, past fp32
+    assert (group4.gated_mlp(x, gate, up, down) == torch.inf).all()
+    x[:, 5] = 2.0 ** 96 * (1.0 - 2.0 ** -12)
+    h = (1.0 - 2.0 ** -12) ** 2 * 2.0 ** 128              # 2^-24 from a whole fp32, and past bf16's largest
+    assert 3.397e38 < h < big
+    # eight equal terms of 2^-10 h: sums and the planes' additions are off by at most 2^-20 together
+    y = group4.gated_mlp(x, gate, up, down).double().cpu()
+    assert ((y / (8 * h * 2.0 ** -10) - 1).abs() < 2.0 ** -20).all()

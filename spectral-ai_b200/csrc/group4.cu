@@ -457,9 +457,13 @@ inline int check_workspace(const void* ws, size_t have, size_t need) {
 // are fed best by the persistent tcgen05 GEMM (gemm_tc.cuh) on weights written out in
 // 16 bits once: N x K x 4 bytes, against M x N x K products.  A value has 13
 // significant bits (a code's 5 times a scale's 8), so it is two bf16 terms exactly,
-// hi + lo, and the sum runs over x hi + x lo: twice the matrix work for the accuracy
-// of the short form, where one rounded term would add as much error as the output's
-// own rounding.  (fp32 activations would take six terms: they stay with the stream.)
+// hi + lo, and the sum runs over x lo + x hi: twice the matrix work, where one rounded
+// term would add as much error as the output's own rounding.  The accumulator
+// truncates every step's sum, so the small terms go first: their steps lose 2^-8 of what
+// they would behind the large ones.  What the large ones' K / 16 steps lose is seen in fp32
+// outputs alone, off by (normwise; in brackets with the large terms first; the short form
+// 0.6 to 1.8e-7) 1.6e-6 (4.3e-6) at K = 2048, 7.7e-6 (2.0e-5) at 8192, 1.6e-5 (4.1e-5) at
+// 16384.  (fp32 activations would take six terms: they stay with the stream.)
 //
 // Which form is the faster one: see long_linear().
 
@@ -496,14 +500,14 @@ __global__ void group4_terms_kernel(const uint8_t* __restrict__ data, bool asym,
   }
 }
 
-// y = x hi + x lo (+ bias): the tokens' K blocks twice
+// y = x lo + x hi (+ bias): the tokens' K blocks twice
 struct EpiGroup4Rows {
   const float* bias;
   void* y;
   int64_t ldo;
   int dtype, N, kb;  // kb: K blocks of a term
   __device__ __forceinline__ int a_block(int i) const { return i < kb ? i : i - kb; }
-  __device__ __forceinline__ int b_block(int i) const { return i; }
+  __device__ __forceinline__ int b_block(int i) const { return i < kb ? i + kb : i - kb; }
   __device__ __forceinline__ void apply(int64_t row, int col0, const uint32_t (&r)[32]) const {
     if (dtype == SB_BF16 && col0 + 32 <= N && (ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0) {
       uint32_t p[16];
@@ -536,7 +540,7 @@ struct EpiGroup4Hidden {
   int64_t ip;
   int I, kb;
   __device__ __forceinline__ int a_block(int i) const { return i < kb ? i : i - kb; }
-  __device__ __forceinline__ int b_block(int i) const { return i; }
+  __device__ __forceinline__ int b_block(int i) const { return i < kb ? i + kb : i - kb; }
   __device__ __forceinline__ void apply(int64_t row, int col0, const uint32_t (&r)[32]) const {
     __nv_bfloat16 hi[16], lo[16];
     const int c0 = col0 / 2;
@@ -559,9 +563,9 @@ struct EpiGroup4Hidden {
   __device__ __forceinline__ void tail(int64_t, const uint32_t (&)[32]) const {}
 };
 
-// y = h_hi w_hi + h_hi w_lo + h_lo w_hi (what is left out, h_lo w_lo, is 2^-16 of it)
+// y = h_lo w_hi + h_hi w_lo + h_hi w_hi (what is left out, h_lo w_lo, is 2^-16 of it)
 struct EpiGroup4Down : EpiGroup4Rows {
-  __device__ __forceinline__ int a_block(int i) const { return i < kb ? i : i - kb; }
+  __device__ __forceinline__ int a_block(int i) const { return i < kb ? i + kb : i < 2 * kb ? i - kb : i - 2 * kb; }
   __device__ __forceinline__ int b_block(int i) const { return i < 2 * kb ? i : i - 2 * kb; }
 };
 

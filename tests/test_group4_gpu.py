@@ -430,3 +430,47 @@ def test_largest_and_infinite_fp32_values(cuda_device, M):
     # eight equal terms of 2^-10 h: sums and the planes' additions are off by at most 2^-20 together
     y = group4.gated_mlp(x, gate, up, down).double().cpu()
     assert ((y / (8 * h * 2.0 ** -10) - 1).abs() < 2.0 ** -20).all()
+
+
+def _term_order_weights(N, K, cuda_device):
+    """Weights of 15 x 129/128 = 15.1171875, in two bf16 terms 15.125 and -2^-7."""
+    from sb200 import group4
+    codes = torch.full((N, K), 15, dtype=torch.uint8, device=cuda_device)
+    scales = torch.full((N, -(-K // 128)), 129 / 128, device=cuda_device)
+    return group4.Group4Matrix.pack(codes, scales, torch.zeros(N, -(-K // 128), dtype=torch.uint8, device=cuda_device))
+
+
+def test_long_prompt_keeps_the_small_terms(cuda_device):
+    """The weights' low terms of a long prompt are added up before the large sum that they would
+    be truncated in: one activation of 2^18 beside 2047 ones.  The low terms' sum, a multiple of
+    2^-7 below 2^12, the high terms', a multiple of 2^-3 below 2^15 before the 2^18, and the
+    exact result's rounding: one step of 2^-23 for that, one for truncating it."""
+    from sb200 import group4
+    M, K, N = 1200, 2048, 1001
+    assert _written_out(M, K, N)
+    w = _term_order_weights(N, K, cuda_device)
+    x = torch.ones(M, K, dtype=torch.bfloat16, device=cuda_device)
+    x[:, -1] = 2.0 ** 18
+    want = (15 * 129 / 128) * (K - 1 + 2.0 ** 18)
+    y = group4.linear(x, w, out_dtype=torch.float32).double()
+    assert ((y / want - 1).abs() <= 2 * 2.0 ** -23).all()
+
+
+def test_long_mlp_keeps_the_small_terms(cuda_device):
+    """The same of the gated MLP: its hidden values are 1 and, last, 2^18 (silu(32) = 32 in fp32),
+    and the tokens' low terms of the gate and up products are exact."""
+    from sb200 import _lib, group4
+    M, H, I = 1500, 512, 2048
+    rows = 2 * M * H + 4 * M * I + 1024
+    assert _lib.load().sb_group4_gated_mlp_workspace_bytes(_lib.SB_BF16, M, H, I) > rows + 8 * H * I
+    codes = torch.full((I, H), 8, dtype=torch.uint8, device=cuda_device)
+    codes[:, 0] = 9
+    scales = torch.full((I, H // 128), 32.0, device=cuda_device)
+    ups = torch.full((I, H // 128), 2.0 ** -5, device=cuda_device)
+    ups[-1] = 2.0 ** 13
+    gate, up = group4.Group4Matrix.pack(codes, scales), group4.Group4Matrix.pack(codes, ups)
+    x = torch.zeros(M, H, dtype=torch.bfloat16, device=cuda_device)
+    x[:, 0] = 1
+    want = (15 * 129 / 128) * (I - 1 + 2.0 ** 18)
+    y = group4.gated_mlp(x, gate, up, _term_order_weights(H, I, cuda_device), out_dtype=torch.float32).double()
+    assert ((y / want - 1).abs() <= 2 * 2.0 ** -23).all()

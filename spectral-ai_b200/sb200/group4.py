@@ -303,6 +303,7 @@ def few_moe(experts, x: torch.Tensor, ids: Optional[torch.Tensor], weights: Opti
         if weights.dtype != torch.float32 or not weights.is_contiguous():
             weights = weights.detach().to(torch.float32).contiguous()
     else:
+        _no_grad(gate_weight, "the gate's weights")
         k, gw, gc = top_k, gate_weight.data_ptr(), _code(gate_weight.dtype, "gate")
     most = max_tokens(k)
     if most < 1:

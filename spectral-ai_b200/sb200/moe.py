@@ -78,7 +78,7 @@ class FewTokenMoE:
         if gate_weight.dtype not in (torch.float32, torch.bfloat16):
             raise RuntimeError(f"gate dtype {gate_weight.dtype} must be float32 or bfloat16")
         self.experts = experts
-        self.gate_weight = gate_weight.detach().contiguous()
+        self.gate_weight = gate_weight.contiguous()
         self.top_k = int(top_k)
         self.norm_topk = bool(norm_topk)
 

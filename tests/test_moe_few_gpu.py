@@ -280,3 +280,17 @@ def test_quantised_layer_as_it_is_used(cuda_device):
     yp, ids, w = layer(prompt, routing=True)
     ref, bound = reference(prompt, ids.cpu().numpy(), w.cpu().numpy(), vals)
     close(yp, ref, bound, "prompt")
+
+
+def test_gate_that_needs_a_gradient_is_refused(cuda_device):
+    """A trained gate (an nn.Linear's weight) gets no gradient here: outside no_grad it raises."""
+    from sb200.moe import FewTokenMoE
+    ex, _ = make_experts("group4", 6, 96, 48, cuda_device)
+    gate = torch.nn.Linear(96, 6, bias=False, device=cuda_device)
+    x = acts(3, 96, torch.bfloat16, cuda_device)
+    layer = FewTokenMoE(ex, gate.weight, 2)
+    with pytest.raises(RuntimeError, match="gradient"):
+        layer(x)
+    with torch.no_grad():
+        y = layer(x)
+    assert torch.equal(y, FewTokenMoE(ex, gate.weight.detach(), 2)(x))

@@ -304,6 +304,10 @@ def few_moe(experts, x: torch.Tensor, ids: Optional[torch.Tensor], weights: Opti
             weights = weights.detach().to(torch.float32).contiguous()
     else:
         _no_grad(gate_weight, "the gate's weights")
+        _check_cuda(gate_weight, "gate_weight", dev)
+        if gate_weight.shape != (E, H):
+            raise RuntimeError(f"gate_weight of shape {tuple(gate_weight.shape)} must be [{E}, {H}]")
+        gate_weight = gate_weight.contiguous()  # (copied only where it is not)
         k, gw, gc = top_k, gate_weight.data_ptr(), _code(gate_weight.dtype, "gate")
     most = max_tokens(k)
     if most < 1:

@@ -57,8 +57,8 @@ class FewTokenMoE:
     """A whole MoE layer for decoding batches: dense gate, softmax, top-k, SwiGLU
     experts and their weighted sum, in three to five kernels (six for fp32 rows).
 
-    ``gate_weight`` [E, H] (fp32 or bf16, an ``nn.Linear`` weight) scores the
-    experts; a token's weights are its ``top_k`` largest softmax probabilities, in
+    ``gate_weight`` [E, H] (fp32 or bf16, an ``nn.Linear`` weight, read as it is at
+    each call) scores the experts; a token's weights are its ``top_k`` largest softmax probabilities, in
     descending order, divided by their sum with ``norm_topk`` (the gate of
     OlmoeTopKRouter and of the hybrid gate's dense part, without rounding the
     logits to the hidden dtype).  ``experts``: ``TernaryExperts`` or
@@ -78,7 +78,7 @@ class FewTokenMoE:
         if gate_weight.dtype not in (torch.float32, torch.bfloat16):
             raise RuntimeError(f"gate dtype {gate_weight.dtype} must be float32 or bfloat16")
         self.experts = experts
-        self.gate_weight = gate_weight.contiguous()
+        self.gate_weight = gate_weight
         self.top_k = int(top_k)
         self.norm_topk = bool(norm_topk)
 

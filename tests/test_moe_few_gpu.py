@@ -294,3 +294,25 @@ def test_gate_that_needs_a_gradient_is_refused(cuda_device):
     with torch.no_grad():
         y = layer(x)
     assert torch.equal(y, FewTokenMoE(ex, gate.weight.detach(), 2)(x))
+
+
+def test_gate_is_read_at_each_call(cuda_device):
+    """A gate whose rows are not contiguous is no snapshot, and one that has changed its
+    device, shape or dtype since the layer was made is refused."""
+    from sb200.moe import FewTokenMoE
+    ex, _ = make_experts("group4", 6, 96, 48, cuda_device)
+    x = acts(3, 96, torch.bfloat16, cuda_device)
+    for gate in (acts(96, 6, torch.float32, cuda_device, seed=3).t(), acts(6, 200, torch.float32, cuda_device, seed=3)[:, :96]):
+        layer = FewTokenMoE(ex, gate, 2)
+        assert torch.equal(layer(x), FewTokenMoE(ex, gate.contiguous(), 2)(x))
+        gate.mul_(-1)
+        assert torch.equal(layer(x), FewTokenMoE(ex, gate.contiguous(), 2)(x))
+    linear = torch.nn.Linear(96, 6, bias=False, device=cuda_device).requires_grad_(False)
+    layer = FewTokenMoE(ex, linear.weight, 2)
+    layer(x)
+    for change, word in ((lambda: linear.half(), "dtype"), (lambda: linear.cpu(), "CUDA"),
+                         (lambda: linear.weight.set_(torch.zeros(5, 96, device=cuda_device)), "shape")):
+        linear.to(cuda_device, torch.float32)
+        change()
+        with pytest.raises(RuntimeError, match=word):
+            layer(x)

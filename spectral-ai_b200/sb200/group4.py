@@ -20,6 +20,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import math
 from typing import Optional
 
 import torch
@@ -27,6 +28,7 @@ import torch
 from . import _lib
 
 GROUPS = (32, 64, 128)
+MAX_WIDTH, MAX_EXPERTS = 8192, 512  # H and I, and E, of the few-token layer
 
 
 _NOWHERE = contextlib.nullcontext()
@@ -125,9 +127,7 @@ class Group4Matrix:
             raise RuntimeError(f"group {group} must be one of {GROUPS}")
         if len(shape) < 2 or min(shape) < 1:
             raise RuntimeError(f"weights of shape {tuple(shape)} must be [..., N, K] and not empty")
-        count = 1
-        for n in shape[:-2]:
-            count *= n
+        count = math.prod(shape[:-2])
         N, K = shape[-2:]
         data = torch.empty(count * _matrix_bytes(K, N, group, zeros), dtype=torch.uint8, device=device)
         return cls(data, N, K, group, zeros, count)
@@ -336,13 +336,22 @@ def few_moe(experts, x: torch.Tensor, ids: Optional[torch.Tensor], weights: Opti
     return y, ids, weights
 
 
+def check_experts(E: int, H: int, I: int) -> None:
+    """Experts that the few-token layer takes."""
+    if E > MAX_EXPERTS or max(H, I) > MAX_WIDTH:
+        raise RuntimeError(f"{E} experts of {H} x {I}: the few-token layer takes up to {MAX_EXPERTS} experts and {MAX_WIDTH} "
+                           "channels each way")
+
+
 class Group4Experts:
     """E SwiGLU experts in 4-bit groups on one device: ``gate`` and ``up`` count E
     matrices [I, H], ``down`` E matrices [H, I], all in groups of one size, with zero
-    points in all three or in none."""
+    points in all three or in none.  E is at most ``MAX_EXPERTS``, H and I ``MAX_WIDTH``
+    (``gated_mlp`` takes single experts of up to 16384)."""
 
     def __init__(self, gate: Group4Matrix, up: Group4Matrix, down: Group4Matrix):
         self.E, self.I, self.H = gate.count, gate.N, gate.K
+        check_experts(self.E, self.H, self.I)
         if (up.count, up.N, up.K) != (self.E, self.I, self.H) or (down.count, down.N, down.K) != (self.E, self.H, self.I):
             raise RuntimeError(f"{gate.count} gate [{gate.N}, {gate.K}], {up.count} up [{up.N}, {up.K}] and {down.count} "
                                f"down [{down.N}, {down.K}] matrices are not experts of one shape")
@@ -359,6 +368,9 @@ class Group4Experts:
     def pack(cls, gate: dict, up: dict, down: dict, group: int = 128) -> "Group4Experts":
         """From codes [E, N, K], scales and (optional) zeros of each kind of matrix, as
         ``Group4Matrix.pack`` takes them."""
+        shape = gate["codes"].shape
+        if len(shape) > 1:
+            check_experts(math.prod(shape[:-2]), shape[-1], shape[-2])
         return cls(*(Group4Matrix.pack(m["codes"], m["scales"], m.get("zeros"), group) for m in (gate, up, down)))
 
     @classmethod
@@ -368,6 +380,7 @@ class Group4Experts:
         for t, what in ((gate, "gate"), (up, "up"), (down, "down")):
             if t.dim() != 3:
                 raise RuntimeError(f"{what} must be [E, N, K], got {tuple(t.shape)}")
+        check_experts(gate.shape[0], gate.shape[2], gate.shape[1])
         return cls(*(quantize(t, group, symmetric) for t in (gate, up, down)))
 
     def memory_bytes(self) -> int:

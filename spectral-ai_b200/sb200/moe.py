@@ -77,6 +77,7 @@ class FewTokenMoE:
             raise RuntimeError(f"top_k {top_k} is not in 1..{min(E, 32)}")
         if gate_weight.dtype not in (torch.float32, torch.bfloat16):
             raise RuntimeError(f"gate dtype {gate_weight.dtype} must be float32 or bfloat16")
+        group4.check_experts(E, H, experts.I)
         self.experts = experts
         self.gate_weight = gate_weight
         self.top_k = int(top_k)

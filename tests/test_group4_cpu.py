@@ -194,3 +194,33 @@ def test_scales_of_data_inside_a_larger_buffer(group, zeros):
         assert part.zeros[N + 17, 0] == data[((1 * 3 + 1) * 3) * block + 1024 + 32 * per + 2]
     else:
         assert part.zeros is None
+
+
+def test_experts_past_the_layers_limits_are_refused_when_made():
+    """Not at the first call, when the weights have been packed; the limits are the kernels' own."""
+    from types import SimpleNamespace
+
+    from sb200.moe import FewTokenMoE
+    E, W = group4.MAX_EXPERTS, group4.MAX_WIDTH
+
+    def few(E, H, I):
+        ex = _lib.Experts(kind=1, n_experts=E, hidden=H, intermediate=I, group=64, gate=P, up=P, down=P, zeros=0)
+        return _lib.load().sb_moe_few(C.byref(ex), P, 1, H, 0, 1, None, 1, 0, P, P, P, 0, P, 1 << 30, None)
+
+    assert few(E, W, W) == 0
+    data = torch.empty(0)
+    for e, h, i in ((E + 1, 64, 32), (4, W + 1, 32), (4, 64, W + 1)):
+        refused(few(e, h, i))
+        mats = [SimpleNamespace(count=e, N=n, K=k, group=64, has_zeros=False, device=data.device, data=data)
+                for n, k in ((i, h), (i, h), (h, i))]
+        with pytest.raises(RuntimeError, match="up to 512 experts and 8192"):
+            group4.Group4Experts(*mats)
+        on_cpu = [torch.empty(e, n, k, device="meta", dtype=torch.uint8) for n, k in ((i, h), (i, h), (h, i))]
+        with pytest.raises(RuntimeError, match="up to 512 experts and 8192"):
+            group4.Group4Experts.quantize(*on_cpu)
+        with pytest.raises(RuntimeError, match="up to 512 experts and 8192"):
+            group4.Group4Experts.pack(*({"codes": t, "scales": t} for t in on_cpu))
+        with pytest.raises(RuntimeError, match="up to 512 experts and 8192"):
+            FewTokenMoE(SimpleNamespace(E=e, H=h, I=i, gate=data), torch.empty(e, h), top_k=1)
+    mats = [SimpleNamespace(count=E, N=W, K=W, group=64, has_zeros=False, device=data.device, data=data) for _ in range(3)]
+    assert group4.Group4Experts(*mats).E == E

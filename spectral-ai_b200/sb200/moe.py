@@ -42,7 +42,8 @@ class BVHMoELayer:
         return self._run(x, ids, w, out_dtype or x.dtype, out)
 
     def _run(self, x, ids, w, out_dtype, out=None) -> torch.Tensor:
-        f = self.experts.forward_few if x.shape[0] <= self.few_tokens else self.experts.forward
+        few = 0 < ids.shape[0] <= self.few_tokens
+        f = self.experts.forward_few if few else self.experts.forward
         return f(x, ids, w, out_dtype=out_dtype, out=out)
 
     __call__ = forward

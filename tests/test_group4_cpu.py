@@ -224,3 +224,28 @@ def test_experts_past_the_layers_limits_are_refused_when_made():
             FewTokenMoE(SimpleNamespace(E=e, H=h, I=i, gate=data), torch.empty(e, h), top_k=1)
     mats = [SimpleNamespace(count=E, N=W, K=W, group=64, has_zeros=False, device=data.device, data=data) for _ in range(3)]
     assert group4.Group4Experts(*mats).E == E
+
+
+def test_which_form_a_batch_takes():
+    """An empty batch is no few-token batch: with few_tokens off nothing goes to forward_few, whose
+    limits are narrower; tokens are counted by their routing."""
+    from sb200.moe import BVHMoELayer
+    from sb200.ternary import TernaryExperts
+
+    class Experts(TernaryExperts):
+        def __init__(self):
+            pass
+
+        def forward(self, x, ids, w, out_dtype=None, out=None):
+            return "grouped"
+
+        def forward_few(self, x, ids, w, out_dtype=None, out=None):
+            return "few"
+
+    def runs(few_tokens, B, lead=()):
+        layer = BVHMoELayer(None, Experts(), device="cpu", few_tokens=few_tokens)
+        return layer.forward_topk(torch.zeros(*(lead or (B,)), 4), torch.zeros(B, 40), torch.zeros(B, 40, dtype=torch.int32))
+
+    assert [runs(0, B) for B in (0, 1, 300)] == ["grouped"] * 3
+    assert [runs(16, B) for B in (0, 1, 16, 17)] == ["grouped", "few", "few", "grouped"]
+    assert runs(16, 24, lead=(2, 12)) == "grouped"

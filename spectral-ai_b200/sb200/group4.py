@@ -86,16 +86,24 @@ def _rows(x: torch.Tensor, K: int, device: torch.device):
     return x, M, max(ld, K)
 
 
-def _output(out, x: torch.Tensor, shape, dtype, device) -> torch.Tensor:
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from one tensor's first to its last element meets the other's."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
+        return False
+    end = lambda t: t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))  # noqa: E731
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+def _output(out, shape, dtype, device, **inputs) -> torch.Tensor:
+    """``out``, checked, or a new tensor; ``inputs`` (by name) are read while it is written."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
     _check_cuda(out, "out", device)
     if tuple(out.shape) != tuple(shape) or not out.is_contiguous():
         raise RuntimeError(f"out must be contiguous of shape {tuple(shape)}, got {tuple(out.shape)}")
-    if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and x.numel():
-        lo, hi = x.data_ptr(), x.data_ptr() + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
-        if out.data_ptr() < hi and lo < out.data_ptr() + out.numel() * out.element_size():
-            raise RuntimeError("out overlaps the activations, which are read while it is written")
+    for what, t in inputs.items():
+        if t is not None and _overlap(out, t):
+            raise RuntimeError(f"out overlaps the {what.replace('_', ' ')}, which are read while it is written")
     return out
 
 
@@ -237,7 +245,7 @@ def linear(x: torch.Tensor, w: Group4Matrix, bias: Optional[torch.Tensor] = None
         _no_grad(bias, "the bias's values")
         if bias.dtype != torch.float32 or not bias.is_contiguous():
             bias = bias.detach().to(torch.float32).contiguous()
-    y = _output(out, x2, (*x.shape[:-1], w.N), out_dtype or x.dtype, dev)
+    y = _output(out, (*x.shape[:-1], w.N), out_dtype or x.dtype, dev, activations=x2, bias_values=bias)
     xc, xp, ws, need = _code(x2.dtype, "activation"), x2.data_ptr(), None, 0
     if xc != _lib.SB_BF16 or w.K % 8 or ldx % 8 or xp % 16 or _linear_bytes(xc, M, w.K, w.N) > 2 * M * w.K + 255:
         need = _linear_bytes(xc, M, w.K, w.N)
@@ -257,7 +265,7 @@ def gated_mlp(x: torch.Tensor, gate: Group4Matrix, up: Group4Matrix, down: Group
     if up.device != dev or down.device != dev:
         raise RuntimeError("gate, up and down must be on one device")
     x2, M, ldx = _rows(x, gate.K, dev)
-    y = _output(out, x2, (*x.shape[:-1], down.N), out_dtype or x.dtype, dev)
+    y = _output(out, (*x.shape[:-1], down.N), out_dtype or x.dtype, dev, activations=x2)
     xc = _code(x2.dtype, "activation")
     need = lib.sb_group4_gated_mlp_workspace_bytes(xc, M, gate.K, gate.N)
     ws = _workspace(need, dev)
@@ -312,7 +320,7 @@ def few_moe(experts, x: torch.Tensor, ids: Optional[torch.Tensor], weights: Opti
     most = max_tokens(k)
     if most < 1:
         raise RuntimeError(f"top_k {k} is not in 1..32")
-    y = _output(out, x2, x.shape, out_dtype or x.dtype, dev)
+    y = _output(out, x.shape, out_dtype or x.dtype, dev, activations=x2, ids=ids, weights=weights, gate_weights=gate_weight)
     yc, n = _code(y.dtype, "output"), min(B, most)
     need = _moe_bytes(xc, n, H, experts.I, E, k)
     if ids is not None:

@@ -249,3 +249,16 @@ def test_which_form_a_batch_takes():
     assert [runs(0, B) for B in (0, 1, 300)] == ["grouped"] * 3
     assert [runs(16, B) for B in (0, 1, 16, 17)] == ["grouped", "few", "few", "grouped"]
     assert runs(16, 24, lead=(2, 12)) == "grouped"
+
+
+def test_overlap():
+    """Where two views of one storage meet, and where they only lie side by side."""
+    b = torch.zeros(100)
+    f = group4._overlap
+    assert f(b[:10], b[9:12]) and f(b[9:12], b[:10]) and f(b, b[50:51]) and f(b[50:51], b)
+    assert not f(b[:10], b[10:12]) and not f(b[10:12], b[:10])
+    assert not f(b[:10], torch.zeros(10)) and not f(b[:0], b) and not f(b, b[5:5])
+    rows = b[:96].view(12, 8)
+    assert f(rows[:, :4], b[4:5]) and not f(rows[:6], rows[6:]) and f(rows[:, 1], b[9:10])
+    assert f(b[:10], b.view(torch.int32)[9:11]) and not f(b[:10], b.view(torch.int16)[20:22])
+    assert f(b[3:4].expand(5), b[3:4]) and not f(b[3:4].expand(5), b[4:5])

@@ -474,3 +474,14 @@ def test_long_mlp_keeps_the_small_terms(cuda_device):
     want = (15 * 129 / 128) * (I - 1 + 2.0 ** 18)
     y = group4.gated_mlp(x, gate, up, _term_order_weights(H, I, cuda_device), out_dtype=torch.float32).double()
     assert ((y / want - 1).abs() <= 2 * 2.0 ** -23).all()
+
+
+def test_out_that_overlaps_the_bias_is_refused(cuda_device):
+    from sb200 import group4
+    w = make(48, 128, 64, False, cuda_device)[0]
+    x = acts(3, 128, torch.bfloat16, cuda_device)
+    buffer = torch.zeros(4, 48, device=cuda_device)
+    with pytest.raises(RuntimeError, match="overlaps the bias"):
+        group4.linear(x, w, buffer[1], out=buffer[:3])
+    y = group4.linear(x, w, buffer[3], out=buffer[:3])
+    assert torch.equal(y, group4.linear(x, w, out_dtype=torch.float32))

@@ -316,3 +316,20 @@ def test_gate_is_read_at_each_call(cuda_device):
         change()
         with pytest.raises(RuntimeError, match=word):
             layer(x)
+
+
+def test_out_that_overlaps_the_routing_or_the_gate_is_refused(cuda_device):
+    from sb200.moe import FewTokenMoE
+    ex, _ = make_experts("group4", 6, 96, 48, cuda_device)
+    x = acts(3, 96, torch.bfloat16, cuda_device)
+    ids, w = (torch.from_numpy(a).to(cuda_device) for a in routing(3, 2, 6, seed=3))
+    buffer = torch.zeros(6 * 96 + 6, device=cuda_device)
+    out, behind = buffer[:3 * 96].view(3, 96), buffer[6 * 96:].view(3, 2)
+    inside = buffer[100:106].view(3, 2)
+    for bad in ((inside.view(torch.int32), w), (ids, inside)):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ex.forward_few(x, *bad, out=out)
+    with pytest.raises(RuntimeError, match="overlaps the gate"):
+        FewTokenMoE(ex, buffer[:6 * 96].view(6, 96), 2)(x, out=out)
+    behind.copy_(w)
+    assert torch.equal(ex.forward_few(x, ids, behind, out=out), ex.forward_few(x, ids, w))

@@ -50,6 +50,7 @@
 #pragma once
 
 #include "sm100.cuh"
+#include "few_ring.cuh"
 #include "gemm_tc.cuh"
 #include "ternary_gemm.cuh"
 
@@ -411,33 +412,44 @@ struct TernaryW {
   __device__ __forceinline__ float out_scale(int64_t r) const { return __ldg(scales + r); }
 };
 
+// Waits for the next slot of a warp's ring.  Where the wait runs out (and is reported), the
+// copies on their way, one for each slot at most and in the slots' order, get the same time
+// once more, so that none lands in shared memory that the block has left.  (No part of the
+// kernels' own code: the registers of a chunk's arithmetic are in use where it is called.)
+__device__ __noinline__ bool few_ring_wait(uint64_t* bars, FewSlots slots) {
+  if (mbar_wait_warp(bars + slots.out, slots.parity, ST_TIMEOUT_PRODUCER)) return true;
+  const uint64_t t0 = globaltimer();
+#pragma unroll 1
+  for (int i = 0; i < slots.depth; ++i) {
+    uint32_t phase;
+    const uint32_t bar = smem_u32(bars + slots.ahead(i, &phase));
+    while (!mbar_test_wait(bar, phase) && globaltimer() - t0 <= SB_WAIT_LIMIT_NS) __nanosleep(1000);
+  }
+  return false;
+}
+
 // A warp's ring: `depth` slots of RT blocks and a barrier each, filled and used in turn.
 template <class W, int RT>
 struct FewRing {
   uint32_t base;
   uint64_t* bars;
-  int depth, out;
-  uint32_t parity;
+  FewSlots slots;
   bool lost;  // a wait ran out: no more waits, no more copies
   static __host__ __device__ constexpr int slot_bytes() { return RT * W::SLOT; }
 
-  __device__ __forceinline__ FewRing(uint8_t* smem, uint64_t* bars_, int warp, int depth_)
-      : base(smem_u32(smem) + warp * depth_ * slot_bytes()), bars(bars_ + warp * depth_), depth(depth_), out(0),
-        parity(0), lost(false) {}
+  __device__ __forceinline__ FewRing(uint8_t* smem, uint64_t* bars_, int warp, int depth)
+      : base(smem_u32(smem) + warp * depth * slot_bytes()), bars(bars_ + warp * depth), slots(depth), lost(false) {}
   __device__ __forceinline__ void fetch(int slot, const W& w, const typename W::Tile (&t)[RT], int c, int lane) {
     if (!lost) w.template fetch<RT>(base + slot * slot_bytes(), bars + slot, t, c, lane);
   }
   // reads the next slot once it has been filled; returns it, free to be filled again
   __device__ __forceinline__ int take(const W& w, typename W::template Part<RT>& p, int lane) {
-    if (!__all_sync(0xffffffffu, mbar_test_wait(smem_u32(bars + out), parity)) && !lost)
-      lost = !mbar_wait_warp(bars + out, parity, ST_TIMEOUT_PRODUCER);
-    const int slot = out;
+    if (!__all_sync(0xffffffffu, mbar_test_wait(smem_u32(bars + slots.out), slots.parity)) && !lost)
+      lost = !few_ring_wait(bars, slots);
+    const int slot = slots.out;
     w.read(p, base + slot * slot_bytes(), lane);
     __syncwarp();
-    if (++out == depth) {
-      out = 0;
-      parity ^= 1u;
-    }
+    slots.taken();
     return slot;
   }
 };

@@ -106,3 +106,12 @@ def moe(x, ids, weights, experts, fp32=False):
             np.add.at(size, t, np.abs(w) * (np.abs(y) + dy))
     # weights are fp32 products, a token's terms are added in up to 8 + k partial sums
     return out, bound + (ids.shape[1] + 16) * STEP * size
+
+
+def planes(v, count):
+    """fp32 values cut into ``count`` bf16 terms, the rest dropped: their sum, as float64."""
+    rest, total = np.asarray(v, np.float64), 0.0
+    for _ in range(count):
+        term = bf16(rest.astype(np.float32))
+        total, rest = total + term, rest - term
+    return total

@@ -275,8 +275,10 @@ int sb_group4_pack(const uint8_t* codes, const void* scales, const uint8_t* zero
 int sb_group4_dequantize(const sb_group4* m, void* out, int out_dtype, void* stream);
 
 /* y[M,N] = x W^T (+ bias fp32 [N], or NULL): x [M,K] SB_F32 or SB_BF16, rows ldx
- * elements apart; y row-major, SB_F32 or SB_BF16; M from 0 to 2^20.  fp32
- * activations keep all their bits (three bf16 terms), sums are fp32.  Products with
+ * elements apart; y row-major, SB_F32 or SB_BF16, apart from every input; M from 0 to
+ * 2^20.  fp32 activations keep all their bits (three bf16 terms), sums are fp32 (of many
+ * bf16 tokens: the tensor cores' truncating ones, off by some 1e-6 per 2048 of K).  A
+ * token with a non-finite value has non-finite outputs, and no other token has.  Products with
  * M N below 2^30 always run (larger ones of fp32 rows may be refused).  The
  * workspace is 256-byte aligned, here and below; this call needs none (NULL) for
  * bf16 x with K and ldx multiples of 8 and x 16-byte aligned, unless the bytes asked
@@ -308,7 +310,7 @@ size_t sb_group4_gated_mlp_workspace_bytes(int x_dtype, int64_t M, int64_t H, in
  * the two agree to rounding).  The hidden state keeps 16 bits for bf16 x, 24 for
  * fp32 x, with fp32's range.  B is at most sb_moe_few_max_tokens(top_k): 256
  * tokens and 2048 (token, slot) pairs; E at most 512, k at most 32, H and I at most
- * 8192. */
+ * 8192.  out lies apart from every input. */
 enum sb_experts_kind { SB_EXPERTS_TERNARY = 0, SB_EXPERTS_GROUP4 = 1 };
 typedef struct {
   int32_t kind;          /* enum sb_experts_kind */

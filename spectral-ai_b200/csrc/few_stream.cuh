@@ -414,8 +414,9 @@ struct TernaryW {
 
 // Waits for the next slot of a warp's ring.  Where the wait runs out (and is reported), the
 // copies on their way, one for each slot at most and in the slots' order, get the same time
-// once more, so that none lands in shared memory that the block has left.  (No part of the
-// kernels' own code: the registers of a chunk's arithmetic are in use where it is called.)
+// once more, so that none lands in shared memory that the block has left.  (A call: as part
+// of the kernels' own code it takes registers from the chunks' arithmetic, 97.4 us for
+// 64 tokens over 4-bit experts against 96.1; without it 94.9.)
 __device__ __noinline__ bool few_ring_wait(uint64_t* bars, FewSlots slots) {
   if (mbar_wait_warp(bars + slots.out, slots.parity, ST_TIMEOUT_PRODUCER)) return true;
   const uint64_t t0 = globaltimer();

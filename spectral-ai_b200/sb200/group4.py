@@ -235,7 +235,8 @@ def _linear_bytes(xc: int, M: int, K: int, N: int) -> int:
 
 def linear(x: torch.Tensor, w: Group4Matrix, bias: Optional[torch.Tensor] = None, out_dtype=None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y[..., N] = x W^T (+ bias), in x's dtype unless ``out_dtype`` (or ``out``) says fp32 or bf16."""
+    """y[..., N] = x W^T (+ bias), in x's dtype unless ``out_dtype`` (or ``out``, which overlaps no
+    input) says fp32 or bf16."""
     lib, dev = _lib.load(), w.device
     x2, M, ldx = _rows(x, w.K, dev)
     if bias is not None:

@@ -276,7 +276,8 @@ int sb_group4_dequantize(const sb_group4* m, void* out, int out_dtype, void* str
 
 /* y[M,N] = x W^T (+ bias fp32 [N], or NULL): x [M,K] SB_F32 or SB_BF16, rows ldx
  * elements apart; y row-major, SB_F32 or SB_BF16, apart from every input; M from 0 to
- * 2^20.  fp32 activations keep all their bits (three bf16 terms), sums are fp32 (of many
+ * 2^20.  fp32 activations keep all their bits (three bf16 terms; fewer below 2^-110, where
+ * the last term is below bf16's smallest), sums are fp32 (of many
  * bf16 tokens: the tensor cores' truncating ones, off by some 1e-6 per 2048 of K).  A
  * token with a non-finite value has non-finite outputs, and no other token has.  Products with
  * M N below 2^30 always run (larger ones of fp32 rows may be refused).  The
